@@ -68,6 +68,15 @@ optional<Tensor> dense(const optional<Tensor>& t) {
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const optional<Tensor>& t) { return t && wants_grad(*t); }
 
+// A tangent is refused: below autograd's keys it would be lost without a word.
+void check_tangent(const char* name, const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), name,
+                                ": forward-mode derivatives are not implemented");
+}
+void check_tangent(const char* name, const optional<Tensor>& t) {
+    if (t) check_tangent(name, *t);
+}
+
 // ---------------------------------------------------------------- layer norm
 void check_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps,
                 at::ScalarType out) {
@@ -205,6 +214,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm_autograd(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps,
                            optional<at::ScalarType> out_dtype) {
+    check_tangent("layer_norm", x);
+    check_tangent("layer_norm", weight);
+    check_tangent("layer_norm", bias);
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
         return LayerNorm::apply(x, weight, bias, eps, out_dtype);
     static const auto op = operation<decltype(layer_norm)>("spmm_amd::layer_norm");
@@ -331,6 +343,7 @@ struct CrossEntropy : torch::autograd::Function<CrossEntropy> {
 };
 
 Tensor cross_entropy_autograd(const Tensor& logits, const Tensor& target, int64_t ignore_index, int64_t reduction) {
+    check_tangent("cross_entropy", logits);
     if (at::GradMode::is_enabled() && wants_grad(logits))
         return CrossEntropy::apply(logits, target, ignore_index, reduction);
     static const auto op = operation<decltype(cross_entropy)>("spmm_amd::cross_entropy");
@@ -338,7 +351,7 @@ Tensor cross_entropy_autograd(const Tensor& logits, const Tensor& target, int64_
     return op.call(logits, target, ignore_index, reduction);
 }
 
-// Its outputs are constants to autograd, the gradient among them.
+// Its outputs are constants to autograd in either mode, the gradient among them.
 std::tuple<Tensor, Tensor> cross_entropy_grad_autograd(const Tensor& logits, const Tensor& target, int64_t ignore_index,
                                                        int64_t reduction, double scale) {
     static const auto op = operation<decltype(cross_entropy_grad)>("spmm_amd::cross_entropy_grad");

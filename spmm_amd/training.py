@@ -11,7 +11,9 @@ so on), defined with their autograd formulas in lib/libtcatorch.so
 (csrc/torch_training.cpp); this module loads it, gives the operators their fake
 kernels (so that torch.compile traces them as opaque nodes) and their Python
 forms.  There is no fallback: without the library the import fails, and tensors
-that are not on a GPU raise ValueError.
+that are not on a GPU raise ValueError.  Derivatives are first derivatives in reverse
+mode: second ones, forward mode (torch.autograd.forward_ad, torch.func.jvp) and
+torch.func.grad raise an error.
 
 Work runs on the current stream of the tensors' device; workspaces come from
 torch's allocator.  No counterpart in the reference, which has no training path.
@@ -133,7 +135,7 @@ def cross_entropy_grad(logits: torch.Tensor, target: torch.Tensor, ignore_index:
 
     The loss is not multiplied by `scale` (a loss scale of 16-bit training); the
     gradient is, before it is rounded to the logits' dtype.  reduction: "mean" or
-    "sum".  Both results are constants to autograd."""
+    "sum".  Both results are constants to autograd, in reverse and in forward mode."""
     return _ops.cross_entropy_grad(logits, target, ignore_index,
                                    _reduction("cross_entropy_grad", reduction, ("mean", "sum")), scale)
 
