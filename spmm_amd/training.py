@@ -234,16 +234,49 @@ class AdamW(torch.optim.Optimizer):
                     state["step"] = step + 1
         return loss
 
+    # settings of torch's AdamW: those that would change a step and what they have to be here, and
+    # those that say how torch computes it
+    _FIXED = {"maximize": False, "amsgrad": False, "differentiable": False, "decoupled_weight_decay": True}
+    _THEIRS = (*_FIXED, "foreach", "fused")
+
+    def _check_loaded(self, state_dict) -> None:
+        """ValueError where a saved state would mean something else here."""
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for name in ("lr", "betas", "eps", "weight_decay"):
+                if name not in saved:
+                    raise ValueError(f"AdamW: the loaded group has no {name}: it is not of an AdamW optimizer")
+            for name, value in self._FIXED.items():
+                if saved.get(name, value) != value:
+                    raise ValueError(f"AdamW: a state with {name}={saved[name]} cannot be loaded: only {name}={value} is "
+                                     "supported")
+            bits = saved.get("state_bits", group["state_bits"])
+            if bits not in self._STATES:
+                raise ValueError(f"AdamW: state_bits must be 32 or 8, got {bits}")
+            for i, p in zip(saved["params"], group["params"]):
+                if not state_dict["state"].get(i):
+                    continue
+                names = {"step", *self._STATES[bits]} | ({"master"} if p.dtype != torch.float32 else set())
+                if set(state_dict["state"][i]) != names:
+                    raise ValueError(f"AdamW: the loaded state of a {p.dtype} parameter must hold {sorted(names)} for states "
+                                     f"in {bits} bits, got {sorted(state_dict['state'][i])}")
+
     def load_state_dict(self, state_dict) -> None:
         """torch.optim.Optimizer.load_state_dict, with the states in their own
         dtypes (the base class casts them to their parameters').  Takes torch's
-        AdamW's for float32 parameters too, whose step counts are tensors."""
+        AdamW's for float32 parameters and 32-bit states too: its step counts are
+        tensors, state_bits and capturable stay this optimizer's, and options that
+        change its step (maximize, amsgrad, differentiable, coupled decay) are refused."""
+        self._check_loaded(state_dict)
+        own = [{name: group[name] for name in ("state_bits", "capturable")} for group in self.param_groups]
         super().load_state_dict(state_dict)
+        for group, settings in zip(self.param_groups, own):
+            if "state_bits" not in group:  # torch's
+                group.update(settings)
+            group.setdefault("capturable", settings["capturable"])
+            for name in self._THEIRS:
+                group.pop(name, None)
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
-        for group in self.param_groups:
-            for name in ("state_bits", "capturable"):
-                group.setdefault(name, self.defaults[name])
         capturable = [group["capturable"] for group in self.param_groups for _ in group["params"]]
         for i, p, c in zip(ids, params, capturable):
             if i not in state_dict["state"]:
