@@ -119,7 +119,8 @@ typedef struct tca_adamw_tensor {
     int64_t n;
 } tca_adamw_tensor;
 
-/* One step over `count` tensors (a HOST array, copied into the launches). */
+/* One step over `count` tensors (a HOST array, copied into the launches).  They are
+ * worked on side by side: no two share memory (TCA_ERR_INVALID if parameters do). */
 int tca_adamw_step(const tca_adamw_tensor* tensors, int32_t count, int32_t param_dtype, int32_t state_bits,
                    int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
                    void* stream);

@@ -1,7 +1,10 @@
 // adamw.hip -- C ABI of the AdamW step (include/tca_train.h).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <utility>
+#include <vector>
 
 #include "../../include/tca_train.h"
 #include "adamw_kernel.hpp"
@@ -48,6 +51,25 @@ int check_tensor(const char* name, const tca_adamw_tensor& t, int k, bool master
     return TCA_OK;
 }
 
+// Two tensors on the same values: the workgroups of a launch would race on them.
+int check_apart(const char* name, const tca_adamw_tensor* tensors, int count, int32_t dtype) {
+    if (count < 2) return TCA_OK;
+    return api_guard(name, [&] {
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;  // [first, past the last) byte
+        spans.reserve(count);
+        for (int k = 0; k < count; ++k) {
+            if (tensors[k].n == 0) continue;
+            const uintptr_t first = reinterpret_cast<uintptr_t>(tensors[k].param);
+            spans.emplace_back(first, first + static_cast<uintptr_t>(tensors[k].n) * dtype_size(dtype));
+        }
+        std::sort(spans.begin(), spans.end());
+        for (size_t k = 1; k < spans.size(); ++k)
+            if (spans[k].first < spans[k - 1].second)
+                return fail(TCA_ERR_INVALID, "%s: two tensors' parameters share memory", name);
+        return static_cast<int>(TCA_OK);
+    });
+}
+
 // Both entry points: step counts of the host (d_steps NULL) or of the device.
 int adam_step(const char* name, const tca_adamw_tensor* tensors, int64_t* const* d_steps, int32_t count,
               int32_t param_dtype, int32_t state_bits, int64_t step, double lr, double beta1, double beta2, double eps,
@@ -64,6 +86,7 @@ int adam_step(const char* name, const tca_adamw_tensor* tensors, int64_t* const*
     const bool bits8 = state_bits == 8, master = param_dtype != TCA_F32;
     for (int k = 0; k < count; ++k)
         if (const int st = check_tensor(name, tensors[k], k, master, bits8, param_dtype)) return st;
+    if (const int st = check_apart(name, tensors, count, param_dtype)) return st;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     AdamArgs a;
     a.keep = static_cast<float>(1.0 - lr * weight_decay);

@@ -174,6 +174,15 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       capturable=capturable))
 
+    def add_param_group(self, param_group) -> None:
+        """torch.optim.Optimizer.add_param_group; a parameter given twice, of which torch
+        only warns, is refused: a launch would update it twice at once."""
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        if len({id(p) for p in params}) != len(params):
+            self.param_groups.pop()
+            raise ValueError("AdamW: a parameter is in its group more than once")
+
     def _new_state(self, p: torch.Tensor, bits: int, capturable: bool) -> dict:
         if not p.is_cuda:
             raise ValueError(f"AdamW: parameters must be GPU tensors (no CPU fallback), got {p.device}")
