@@ -165,23 +165,30 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, capturable: bool = False):
+        self._check_settings(lr, betas, eps, weight_decay, state_bits)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      capturable=capturable))
+
+    def _check_settings(self, lr, betas, eps, weight_decay, state_bits) -> None:
         if state_bits not in self._STATES:
             raise ValueError(f"AdamW: state_bits must be 32 or 8, got {state_bits}")
         if not (eps >= 0 and lr >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
             raise ValueError(f"AdamW: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
         if state_bits == 8 and not eps > 0:
             raise ValueError("AdamW: states in 8 bits need eps above 0")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      capturable=capturable))
 
     def add_param_group(self, param_group) -> None:
         """torch.optim.Optimizer.add_param_group; a parameter given twice, of which torch
         only warns, is refused: a launch would update it twice at once."""
         super().add_param_group(param_group)
-        params = self.param_groups[-1]["params"]
-        if len({id(p) for p in params}) != len(params):
+        group = self.param_groups[-1]
+        try:
+            self._check_settings(*(group[name] for name in ("lr", "betas", "eps", "weight_decay", "state_bits")))
+            if len({id(p) for p in group["params"]}) != len(group["params"]):
+                raise ValueError("AdamW: a parameter is in its group more than once")
+        except ValueError:
             self.param_groups.pop()
-            raise ValueError("AdamW: a parameter is in its group more than once")
+            raise
 
     def _new_state(self, p: torch.Tensor, bits: int, capturable: bool) -> dict:
         if not p.is_cuda:

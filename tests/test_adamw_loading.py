@@ -97,3 +97,15 @@ def test_a_wrong_number_of_parameters_is_torchs_refusal():
     saved["param_groups"][0]["params"] = [0]
     with pytest.raises(ValueError):
         T.AdamW(_params()).load_state_dict(saved)
+
+
+@pytest.mark.parametrize("settings", [dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0),
+                                      dict(state_bits=8, eps=0.0), dict(weight_decay=-0.1)])
+def test_a_groups_own_settings_are_checked(settings):
+    p, q = _params()
+    with pytest.raises(ValueError, match="AdamW"):
+        T.AdamW([dict(params=[p], **settings)])
+    opt = T.AdamW([p])
+    with pytest.raises(ValueError, match="AdamW"):
+        opt.add_param_group(dict(params=[q], **settings))
+    assert len(opt.param_groups) == 1
