@@ -57,6 +57,7 @@ int tca_layer_norm_backward(const void* d_dy, int64_t dy_pitch, int32_t y_dtype,
  * [0, classes) that is not ignore_index gives NaN in the loss and in its
  * row's gradient.  Logits of -inf take no part; a row of nothing else has no
  * distribution and gives NaN.
+ * rows and pitch are below 2^31, classes at most 2^30.
  * reduction: TCA_LOSS_NONE (d_loss [rows]), TCA_LOSS_SUM or TCA_LOSS_MEAN
  * (d_loss [1]; the mean is over the rows that count, and 0 over none). */
 #define TCA_LOSS_NONE 0

@@ -239,6 +239,8 @@ struct LossInput {
         TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == logits.size(0), name, ": target must be 1-D with ",
                           logits.size(0), " entries, got ", t.sizes());
         x = as_rows(logits);
+        // rows further apart than the library takes: their copy holds the rows alone
+        if (x.stride(0) > INT32_MAX) x = x.clone(at::MemoryFormat::Contiguous);
         target = t.contiguous();
     }
     int64_t rows() const { return x.size(0); }
