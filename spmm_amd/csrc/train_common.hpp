@@ -53,6 +53,10 @@ __device__ __forceinline__ T from_f32(float x) {
     if constexpr (sizeof(T) == 4) {
         return x;
     } else if constexpr (__is_same(T, _Float16)) {
+        // x is an fp32 value first: without this the compiler turns some FMAs and their
+        // conversion into one instruction that rounds once, in some places of a kernel
+        // and not in others, and a row's bits depend on its place among the rows
+        asm("" : "+v"(x));
         return static_cast<_Float16>(x);
     } else {
         return __builtin_bit_cast(bf16_t, static_cast<__bf16>(x));  // v_cvt_pk_bf16_f32: nearest even
