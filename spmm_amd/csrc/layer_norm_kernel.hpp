@@ -6,12 +6,15 @@
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
 // Both directions are bound by HBM: a row is read once into registers, its
-// statistics are sums over the team of lanes that holds it (the mean first,
-// then the squared distances from it: no cancellation), and the result is
-// written from the registers.  2.4M rows of 128 fp32 values: forward 445 us
-// (5.7 TB/s), backward 665 us (5.7 TB/s) and 5 us to join the partial sums of dw
-// and db; 8192 rows of 4096 bf16 values forward 24 us (5.5 TB/s).  A copy of 1 GiB
-// reaches 5.1 TB/s.
+// statistics are sums over the team of lanes that holds it, and the result is
+// written from the registers.  The mean is taken twice, as the sum's and as the
+// mean of the distances from that, which a row's size no longer rounds: a row of one
+// value v has mean v and variance 0, not v times the roundings of its sum (at 15
+// values of 1e4, once 0.3 of a deviation beside 0).  The squared distances from
+// it follow.  The third sum costs nothing where HBM bounds, and 0.2 us on a single
+// row.  2.4M rows of 128 fp32 values: forward 446 us (5.6 TB/s), backward 662 us
+// (5.7 TB/s) and 5 us to join the partial sums of dw and db; 8192 rows of 4096 bf16
+// values forward 24 us (5.6 TB/s).  A copy of 1 GiB reaches 5.1 TB/s.
 //
 // FMAs are written out and others forbidden, so the rows' bits do not depend on
 // which variant of a kernel takes them, that is on how many rows there are.
@@ -80,17 +83,23 @@ __global__ __launch_bounds__(team_threads(G)) void layer_norm_kernel(LayerNormAr
         }
         float mean[R], s[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            s[r] = 0.0f;
+        for (int r = 0; r < R; ++r) mean[r] = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v)
+        for (int turn = 0; turn < 2; ++turn) {  // the sum's mean, then what it is off by
 #pragma unroll
-                for (int i = 0; i < E; ++i) s[r] += col.counts(v, i) ? to_f32(raw[r][v].v[i]) : 0.0f;
+            for (int r = 0; r < R; ++r) {
+                s[r] = 0.0f;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) s[r] += col.counts(v, i) ? to_f32(raw[r][v].v[i]) - mean[r] : 0.0f;
+            }
+            sum(s);
+#pragma unroll
+            for (int r = 0; r < R; ++r) mean[r] += s[r] * a.inv_n;
         }
-        sum(s);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            mean[r] = s[r] * a.inv_n;
             s[r] = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v)
