@@ -15,11 +15,14 @@ namespace tca {
 namespace {
 
 // Arrays of more than this are streamed past the caches (256 MB behind the L2s).
-// Where one state is stepped over and over with nothing between, that pays from
-// 256 MB up (16M parameters in fp32, 268 MB: 59 us cached, 76 streamed; 20M: 97 and
-// 94; 134M: 693 and 617; 8-bit states 381 and 305).  Between the steps of a
-// training program its other passes go through the caches, so half of them is
-// the bound.
+// Where one state is stepped over and over with nothing between, that pays only from
+// 384 MB on (fp32 parameters, 16 bytes each in all arrays: 8M 35 us cached, 41
+// streamed; 16M 67 and 83; 24M 129 and 128; 134M 693 and 617; 8-bit states 381 and
+// 305).  In a training program other passes go through the caches between two steps,
+// and then it pays at each of these sizes: with a copy of 256 MB between, copy and
+// step of 8M take 154 us cached, 150 streamed, of 16M 199 and 193, of 48M 364 and 356;
+// with the gradients written before the step and the parameters read after it as well
+// 170 and 166, 222 and 219, 484 and 460.  Half of what the caches hold is the bound.
 constexpr int64_t kAdamStreamBytes = 128ll << 20;
 
 template <typename T, bool kStream>

@@ -67,8 +67,13 @@ int go_from(const CrossEntropyArgs& a, int nv, hipStream_t s) {
 // overhead per value (233k rows of 41 fp32 logits 24 us with one, 20 with two).  A
 // wavefront per row needs no barrier (20000 x 2500 bf16 logits 38 us, 61 with a
 // workgroup of 256); beyond six vectors per lane two wavefronts share a row
-// (20000 x 5000 fp16, forward: 44 us, 61 with one, 54 with four), and eight from
-// 1024 vectors on.
+// (20000 x 5000 fp16, forward: 44 us, 61 with one, 54 with four).  From 1024 vectors
+// on, loss and gradient at once take eight (20000 rows of 5000, 7000 and 10000 bf16
+// logits: 87, 118 and 167 us with two, 106, 113 and 155 with eight) up to sixteen
+// vectors per lane, all that the registers hold (4194 x 50001: 198 us, 212 in the long
+// kernel), and a single direction takes the long kernel (20000 x 10000, backward:
+// 144 us, 169 with two wavefronts; forward, where two would still be ahead up to 1536
+// vectors, 89 and 66).
 template <typename T, int kMode>
 int launch_loss(const CrossEntropyArgs& a, hipStream_t s) {
     constexpr int E = 16 / sizeof(T);

@@ -54,7 +54,8 @@ __device__ __forceinline__ int64_t load_target(const CrossEntropyArgs& a, int64_
 }
 
 // exp(d): the hardware's exp2 of d log2(e).  The product's rounding is relative to
-// |d|, and so is the result's error: largest where exp(d), d <= 0, is smallest.
+// |d|, and so is the result's error, |d| 2^-24: largest where exp(d), d <= 0, is
+// smallest.  Results below 2^-126 are 0.
 // (One FMA, x log2(e) - m log2(e), saves an instruction and overflows for logits
 // near fp32's ends, which masks use.)
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }

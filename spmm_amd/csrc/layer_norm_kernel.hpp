@@ -9,12 +9,11 @@
 // statistics are sums over the team of lanes that holds it, and the result is
 // written from the registers.  The mean is taken twice, as the sum's and as the
 // mean of the distances from that, which a row's size no longer rounds: a row of one
-// value v has mean v and variance 0, not v times the roundings of its sum (at 15
-// values of 1e4, once 0.3 of a deviation beside 0).  The squared distances from
-// it follow.  The third sum costs nothing where HBM bounds, and 0.2 us on a single
-// row.  2.4M rows of 128 fp32 values: forward 446 us (5.6 TB/s), backward 662 us
+// value v has mean v and variance 0 (from the sum alone 15 values of 1e4 came out at
+// -0.3).  The squared distances from it follow.  The third sum costs nothing where HBM bounds, and 0.2 us on a single
+// row.  2.4M rows of 128 fp32 values: forward 449 us (5.6 TB/s), backward 665 us
 // (5.7 TB/s) and 5 us to join the partial sums of dw and db; 8192 rows of 4096 bf16
-// values forward 24 us (5.6 TB/s).  A copy of 1 GiB reaches 5.1 TB/s.
+// values forward 25 us (5.4 TB/s).  A copy of 1 GiB reaches 5.1 TB/s.
 //
 // FMAs are written out and others forbidden, so the rows' bits do not depend on
 // which variant of a kernel takes them, that is on how many rows there are.

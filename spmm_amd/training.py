@@ -147,7 +147,9 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters are contiguous GPU tensors in float32, float16 or bfloat16.  16-bit
     ones have a float32 master copy in the state, which the step updates and
-    rounds into the parameter.  Arithmetic is float32.
+    rounds into the parameter.  Arithmetic is float32.  Gradients are taken as they are:
+    no factor undoes a loss scale, and no step is skipped for a gradient that is not
+    finite.
 
     state_bits 32: state[p] holds "step" (int), "exp_avg" and "exp_avg_sq"
     (float32, p's shape), and "master" (float32) for 16-bit p.
